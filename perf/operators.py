@@ -285,19 +285,13 @@ def _plain_attend(s):
 _PLAIN = {"qk_norm": _plain_qk_norm, "append": _plain_append, "attend": _plain_attend}
 
 
-_loaded = None
-
-
 def _package():
-    global _loaded
-    if _loaded is None:
-        here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fast-moss-tokenizer_b200")
-        if here not in sys.path:
-            sys.path.insert(0, here)
-        import fast_moss_b200
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fast-moss-tokenizer_b200")
+    if here not in sys.path:
+        sys.path.insert(0, here)
+    import fast_moss_b200
 
-        _loaded = fast_moss_b200
-    return _loaded
+    return fast_moss_b200
 
 
 def run(state):
