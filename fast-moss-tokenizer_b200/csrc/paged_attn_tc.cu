@@ -867,6 +867,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st32(o_at + i, o);
             }
+            // a step may rescale twice (raised, then far above the reference all the
+            // same): the second loads follow these stores only where they have landed
+            tmem_st_wait();
             l *= f;
           };
           auto maximum = [&] {

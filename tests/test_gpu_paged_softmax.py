@@ -1,0 +1,95 @@
+"""GPU: the softmax of `paged_attention` over scores that leap from tile to
+tile, against plain float64 evaluations.
+
+The kernels take weights against a reference that they move late: by the
+running maximum once it is exceeded by 2^8 (few rows; d = 64), or raised by a
+power of two when a tile's weights passed 2^16 and by the true maximum when
+they passed 2^100 (d = 128, many rows).  Every such path is reached here: rows
+of all kinds lie side by side in one warp, so that a step takes several of
+them at once.
+
+Bars: as in test_gpu_paged.py, a weight is off by 2^-15 of itself (two bf16
+terms) or 2^-8 more (one term), the result is rounded by 2^-8 of its value; and
+the exponents reach 256 here, see `leaping_scores`.
+"""
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import History, attention_reference, no_device_error
+
+pytestmark = pytest.mark.gpu
+
+# The exponent (base 2) of all keys of tile 0, 1, ... of 128 positions.
+PROFILES = [
+    [0] * 12,
+    [0, 30, 30, 30, 30, 30, 30, 30, 30, 30, 30, 30],            # passes 2^16 once
+    [0, 0, 130, 130, 130, 130, 130, 130, 130, 130, 130, 130],   # passes 2^100 once
+    [0, 22, 44, 66, 88, 110, 132, 154, 176, 198, 220, 242],     # 2^16 in every tile
+    [0, 120, 0, 0, 120, 121, 0, 0, 0, 120, 0, 121],             # up and down again
+    [0, 126, 252, 252, 252, 252, 252, 252, 252, 252, 252, 252],
+    [0, -30, -60, -90, -120, -150, -180, -210, -240, -240, -240, -240],
+    [0, 60, 60, 190, 190, 220, 250, 250, 250, 250, 250, 250],   # both kinds of leap
+    [-250, -250, -130, -100, -70, 30, 40, 170, 200, 200, 201, 250],
+    [0, 17, 16, 33, 34, 50, 67, 83, 100, 203, 219, 236],        # at the limits
+]
+
+
+def leaping_scores(h, q_heads, scale, g):
+    """Queries that pick a profile each (row % len), keys whose first columns
+    hold the profiles' exponents, and unit noise in the others.
+
+    All of it is in bf16: the exponents are integers up to 256, so q . k is
+    off by the float32 accumulation alone, at most 8 * 2^-24 of 300 (exponent
+    and noise); the product with the scale and the shift by the reference by
+    3 * 2^-24 of it.  A weight, and the sum that divides it, is off by ln 2 times
+    that: 2 * 11 * 2^-24 * 300 * ln 2 < 2^-11.9."""
+    hkv, d = h.k.shape[1], h.k.shape[3]
+    count = len(PROFILES)
+    device = h.k.device
+    table = torch.tensor(PROFILES, device=device, dtype=torch.float32)
+    for s, length in enumerate(h.length):
+        at = torch.arange(length, device=device)
+        page, slot = h.where(s, at)
+        column = table[:, (at // 128).clamp(max=11)].T.to(torch.bfloat16)
+        for head in range(hkv):
+            h.k[page, head, slot, :count] = column
+    q = torch.randn(h.n, q_heads, d, generator=g).to(device) * 0.3 / scale / d ** 0.5
+    q[..., :count] = 0
+    row = torch.arange(h.n * q_heads, device=device).view(h.n, q_heads)
+    # with a scale of ln 2 the exponents are those of 2
+    q.scatter_(2, (row % count)[..., None], 1.0)
+    return q.to(torch.bfloat16)
+
+
+SCALE = float(torch.tensor(math.log(2.0), dtype=torch.float32))
+
+
+def check(h, q, got, context, one_term):
+    want, size = attention_reference(h, q, context, SCALE)
+    weight = 2.0 ** -15 + 2.0 ** -11.9 + (2.0 ** -8 if one_term else 0.0)
+    bound = (2.0 ** -8 * want.abs() + weight * size) * 1.001 + 1e-38
+    worst = ((got.double() - want).abs() / bound).max().item()
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,past,hq,hkv,context", [
+    ([200], [1100], 2, 2, 0),           # few items: every one cut and joined
+    ([200], [1100], 2, 2, 300),         # rows that start late
+    ([256], [1000], 150, 150, 0),       # as many items as workers: long pieces
+    ([70, 256], [1300, 700], 160, 40, 400),
+    ([3], [1400], 4, 2, 0),             # few rows
+    ([7] * 30, [40 * i for i in range(30)], 20, 20, 0),
+])
+def test_leaping_scores(moss, cuda_device, d, new, past, hq, hkv, context):
+    g = torch.Generator().manual_seed(d + len(new))
+    h = History(new, past, hkv, d, 32, cuda_device, seed=hq)
+    q = leaping_scores(h, hq, SCALE, g)
+    got = moss.paged_attention(q, h.k, h.v, *h.index, scale=SCALE, context=context or None)
+    no_device_error()
+    check(h, q, got, context, max(new) * (hq // hkv) > 16)
+    again = moss.paged_attention(q, h.k, h.v, *h.index, scale=SCALE, context=context or None)
+    assert torch.equal(again, got)
