@@ -5,8 +5,8 @@ Usage: python build.py [--force]
 
 Both are written next to the Python package (fast_moss_b200/) so that they
 are found without any installation step and travel with the source tree.  The
-library needs only the CUDA runtime; the binding needs torch's and Python's
-headers.
+library comes first and needs only the CUDA toolkit; the binding needs torch's
+and Python's headers, and is left out where torch is not installed.
 """
 
 import argparse
@@ -60,7 +60,7 @@ def inputs():
     return files
 
 
-def up_to_date(target=LIB, files=None):
+def up_to_date(target, files=None):
     if not os.path.exists(target):
         return False
     built = os.path.getmtime(target)
@@ -76,11 +76,14 @@ def _run(cmd, verbose):
         raise RuntimeError(f"{os.path.basename(cmd[0])} failed to build fast_moss_b200")
 
 
-def binding_command(out):
+def torch_directory():
+    """Where torch is installed, None where it is not (it is not imported)."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
-        raise RuntimeError("torch not found; the package's native calls are built against it")
-    torch = os.path.dirname(spec.origin)
+    return os.path.dirname(spec.origin) if spec and spec.origin else None
+
+
+def binding_command(out):
+    torch = torch_directory()
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
     headers = [os.path.join(torch, "include"), os.path.join(cuda, "include"), INCLUDE,
                sysconfig.get_paths()["include"]]
@@ -98,11 +101,19 @@ def build_binding(force=False, verbose=False):
 
 
 def build(force=False, verbose=False):
-    """Compiles the CUDA sources into the shared library, and the binding;
-    returns the library's path."""
-    build_binding(force, verbose)
-    if not force and up_to_date():
-        return LIB
+    """Compiles the CUDA sources into the shared library, and the binding where
+    torch is installed; returns the library's path."""
+    if force or not up_to_date(LIB):
+        build_library(verbose)
+    if torch_directory():
+        build_binding(force, verbose)
+    else:
+        sys.stderr.write("torch not found: the library is built, the Python package's native "
+                         "calls are not\n")
+    return LIB
+
+
+def build_library(verbose=False):
     tmp = LIB + ".tmp"
     with tempfile.TemporaryDirectory() as work:
         objects = [os.path.join(work, s[:-3] + ".o") for s in SOURCES]
@@ -115,7 +126,6 @@ def build(force=False, verbose=False):
             list(pool.map(lambda cmd: _run(cmd, verbose), compiles))
         _run([nvcc_path(), *NVCC_FLAGS, "-shared", *objects, "-o", tmp], verbose)
     os.replace(tmp, LIB)
-    return LIB
 
 
 if __name__ == "__main__":
