@@ -1,5 +1,5 @@
 """Builds libfast_moss_b200.so (sm_100a) in-tree with nvcc, and the package's
-native calls (_binding.so) with the host compiler.
+native calls (_binding-<torch>-<python>.so) with the host compiler.
 
 Usage: python build.py [--force]
 
@@ -12,6 +12,7 @@ and Python's headers, and is left out where torch is not installed.
 import argparse
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -22,9 +23,9 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
-LIB = os.path.join(HERE, "fast_moss_b200", "libfast_moss_b200.so")
+PACKAGE = os.path.join(HERE, "fast_moss_b200")
+LIB = os.path.join(PACKAGE, "libfast_moss_b200.so")
 BINDING_SOURCE = os.path.join(CSRC, "binding.cpp")
-BINDING = os.path.join(HERE, "fast_moss_b200", "_binding.so")
 SOURCES = ["capi.cu", "layer_norm.cu", "rope.cu", "gated_act.cu", "lfq.cu", "rvq.cu",
            "rvq_tc.cu", "rvq_pair.cu", "rvq_noalloc.cu", "qkv_rope.cu", "history_attn.cu", "linear.cu",
            "lfq_rvq.cu", "qk_norm_rope.cu", "paged_attn.cu", "paged_attn_tc.cu"]
@@ -82,6 +83,18 @@ def torch_directory():
     return os.path.dirname(spec.origin) if spec and spec.origin else None
 
 
+def torch_version():
+    """torch.__version__ of the installed torch, which is not imported."""
+    with open(os.path.join(torch_directory(), "version.py")) as f:
+        return re.search(r"^__version__ *= *['\"]([^'\"]+)", f.read(), flags=re.M).group(1)
+
+
+def binding_path():
+    """The binding's file.  It is built against one torch and one Python and
+    fits no other, so it is named for both (fast_moss_b200._lib.binding_path)."""
+    return os.path.join(PACKAGE, f"_binding-{torch_version()}-{sys.implementation.cache_tag}.so")
+
+
 def binding_command(out):
     torch = torch_directory()
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
@@ -95,9 +108,10 @@ def binding_command(out):
 
 def build_binding(force=False, verbose=False):
     files = [BINDING_SOURCE, os.path.join(INCLUDE, "fast_moss_b200.h"), os.path.abspath(__file__)]
-    if force or not up_to_date(BINDING, files):
-        _run(binding_command(BINDING + ".tmp"), verbose)
-        os.replace(BINDING + ".tmp", BINDING)
+    target = binding_path()
+    if force or not up_to_date(target, files):
+        _run(binding_command(target + ".tmp"), verbose)
+        os.replace(target + ".tmp", target)
 
 
 def build(force=False, verbose=False):

@@ -8,7 +8,9 @@ RuntimeError otherwise).
 """
 
 import ctypes
+import importlib.util
 import os
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfast_moss_b200.so")
@@ -138,17 +140,27 @@ def call(name, *args):
 _binding = None
 
 
+def binding_path():
+    """The native binding built against this torch and this Python (build.py)."""
+    import torch
+
+    return os.path.join(HERE, f"_binding-{torch.__version__}-{sys.implementation.cache_tag}.so")
+
+
 def binding():
     """The native calls of the operators that small uses leave bound by the
     host (csrc/binding.cpp), on this library's entry points."""
     global _binding
     if _binding is None:
         lib = load()
-        try:
-            from . import _binding as native
-        except ImportError as e:
-            raise ImportError("fast_moss_b200 native binding not built; run "
-                              "`python fast-moss-tokenizer_b200/build.py`") from e
+        path = binding_path()
+        if not os.path.exists(path):
+            raise ImportError(
+                f"fast_moss_b200 native binding not built for this torch and Python ({path}); run "
+                "`python fast-moss-tokenizer_b200/build.py`")
+        spec = importlib.util.spec_from_file_location(__package__ + "._binding", path)
+        native = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(native)
         native.init(check, *(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                              for name in ("moss_qk_norm_rope", "moss_rope_paged_kv",
                                           "moss_paged_attention",

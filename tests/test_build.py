@@ -53,3 +53,35 @@ def test_the_library_comes_first(native_build, monkeypatch, tmp_path):
     with pytest.raises(RuntimeError):
         native_build.build(force=True)
     assert os.path.exists(native_build.LIB)
+
+
+def test_the_binding_is_that_of_this_torch_and_python(native_build):
+    """Build and package agree on the file, which names both versions."""
+    import sys
+
+    import torch
+    from fast_moss_b200 import _lib
+
+    path = _lib.binding_path()
+    assert native_build.binding_path() == path and os.path.exists(path)
+    assert str(torch.__version__) in path and sys.implementation.cache_tag in path
+
+
+def test_another_torch_gets_a_binding_of_its_own(native_build, monkeypatch, tmp_path):
+    """A binding made for one torch is neither taken for up to date nor loaded
+    under another one."""
+    import torch
+    from fast_moss_b200 import _lib
+
+    monkeypatch.setattr(native_build, "PACKAGE", str(tmp_path))
+    native_build.build_binding()
+    native_build.build_binding()
+    assert len(native_build.ran) == 1
+    monkeypatch.setattr(native_build, "torch_version", lambda: "99.0")
+    native_build.build_binding()
+    assert len(native_build.ran) == 2 and "99.0" in native_build.binding_path()
+
+    monkeypatch.setattr(_lib, "_binding", None)
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    with pytest.raises(ImportError, match="99.0"):
+        _lib.binding()
