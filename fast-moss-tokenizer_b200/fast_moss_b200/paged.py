@@ -79,7 +79,8 @@ class PagedHistory:
       q_start                 int64 [sequences + 1], rows of the step in progress
       kv_len                  int64 [sequences], positions with that step
 
-    A sequence holds at most `max_positions` positions.
+    A sequence holds at most `max_positions` positions.  `lengths` and `rows` are
+    kv_len and q_start[-1] as the host knows them.
     """
 
     def __init__(self, layers, sequences, heads, head_dim, device, *, pages, max_positions,
@@ -104,6 +105,7 @@ class PagedHistory:
         self.q_start = torch.zeros(sequences + 1, device=device, dtype=torch.int64)
         self.kv_len = torch.zeros(sequences, device=device, dtype=torch.int64)
         self.lengths = [0] * sequences
+        self.rows = 0
         self._free = list(range(pages - 1, -1, -1))
         self._pages = [{} for _ in range(sequences)]  # column -> page
         self._changed = {}  # entries of page_table (flat) that the device lacks
@@ -143,6 +145,7 @@ class PagedHistory:
                 self._changed[s * self.page_table.shape[1] + c] = page
             self.lengths[s] += n
             start.append(start[-1] + n)
+        self.rows = start[-1]
         with torch.inference_mode():
             if self._changed:
                 device = self.page_table.device
@@ -152,7 +155,7 @@ class PagedHistory:
                 self._changed.clear()
             self.q_start.copy_(torch.tensor(start))
             self.kv_len.copy_(torch.tensor(self.lengths))
-        return start[-1]
+        return self.rows
 
     def _behind_window(self):
         """Columns of every sequence whose positions no later token attends to."""

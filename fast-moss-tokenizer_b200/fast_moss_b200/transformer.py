@@ -416,16 +416,20 @@ class StreamingTransformer:
         """One step of the streams of a paged history, after `hist.advance(new)`
         made room for their new tokens: x [rows, dim] FP32, the new tokens of
         all streams packed row after row (sum(new) rows; further rows come back
-        undefined and affect no other).  Returns the FP32 residual stream.  max_tokens: an upper
-        bound of new[s], if known.  Reads nothing on the host, so a step of a
-        given number of rows can be captured and replayed after every
-        `advance`."""
+        undefined and affect no other, fewer are refused: the history would
+        count tokens that never came).  Returns the FP32 residual stream.
+        max_tokens: an upper bound of new[s], if known.  Reads nothing of the
+        device, so a step of a given number of rows can be captured and
+        replayed after every `advance`."""
         cfg = self.cfg
         if x.ndim != 2 or x.shape[1] != cfg.dim or x.dtype != torch.float32 or \
                 x.device != self.device:
             raise ValueError("expected [rows, dim] FP32 tokens on the stack's device")
         if len(hist.k_pages) != cfg.layers:
             raise ValueError("the history is of another stack")
+        # (a captured step runs later, on the rows of its replays)
+        if x.shape[0] < hist.rows and not torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"expected the {hist.rows} rows that the history made room for")
         n, h, dh = x.shape[0], cfg.heads, cfg.head_dim
         first = self.layers[0]
         x = x.contiguous()

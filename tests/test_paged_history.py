@@ -99,3 +99,38 @@ def test_stack_config_weight_names():
     assert set(init_weights(normed)[0]) == set(WEIGHT_NAMES) | {"q_norm_w", "k_norm_w"}
     a, b = init_weights(plain, seed=4)[0], init_weights(normed, seed=4)[0]
     assert all(torch.equal(a[k], b[k]) for k in WEIGHT_NAMES)
+
+
+def test_a_step_takes_at_least_the_rows_that_were_made_room_for():
+    """Fewer rows than advance() announced would leave positions of the history
+    unwritten: refused before anything runs; a captured step takes the history
+    as it is at its replays."""
+    from unittest import mock
+
+    from fast_moss_b200 import transformer
+
+    # a stack without its weights, which live on a GPU: nothing here comes to them
+    cfg = transformer.StackConfig(layers=2, dim=128, heads=2, ffn=128, context=8)
+    stack = object.__new__(transformer.StreamingTransformer)
+    stack.cfg, stack.device = cfg, torch.device("cpu")
+    stack.layers = [{"norm1_w": None, "norm1_b": None}] * 2
+    h = stack.paged_history(2, pages=6, max_positions=64)
+    h.advance([5, 1])
+    ran = RuntimeError("the step ran")
+    with mock.patch.object(transformer, "layer_norm", side_effect=ran), \
+            mock.patch.object(torch.cuda, "is_current_stream_capturing", return_value=False):
+        for rows in (0, 1, 5):
+            with pytest.raises(ValueError, match="rows"):
+                stack.step_paged(torch.zeros(rows, 128), h)
+        for rows in (6, 7):
+            with pytest.raises(RuntimeError, match="the step ran"):
+                stack.step_paged(torch.zeros(rows, 128), h)
+        with mock.patch.object(torch.cuda, "is_current_stream_capturing", return_value=True):
+            with pytest.raises(RuntimeError, match="the step ran"):
+                stack.step_paged(torch.zeros(2, 128), h)
+        h.advance([0, 1])
+        with pytest.raises(RuntimeError, match="the step ran"):
+            stack.step_paged(torch.zeros(1, 128), h)
+    with pytest.raises(RuntimeError, match="pages"):
+        h.advance([59, 62])
+    assert h.rows == 1
