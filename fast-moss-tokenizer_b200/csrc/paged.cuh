@@ -38,9 +38,11 @@ struct Seq {
 };
 
 // The sequence's rows and length, clamped so that nothing later leaves the
-// buffers whatever the device arrays hold.
+// buffers whatever the device arrays hold.  Of rows that pass the packed ones
+// those that are there keep their positions.
 __host__ __device__ inline Seq load_seq(const Batch& b, int s) {
   int64_t r0 = b.q_start[s], r1 = b.q_start[s + 1], len = b.kv_len[s];
+  len = (len < 0 ? 0 : len) - (r1 > b.n ? r1 - b.n : 0);
   r0 = r0 < 0 ? 0 : (r0 > b.n ? b.n : r0);
   r1 = r1 < r0 ? r0 : (r1 > b.n ? b.n : r1);
   const int64_t cap = capacity(b);

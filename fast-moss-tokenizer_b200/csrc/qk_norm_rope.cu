@@ -312,6 +312,11 @@ __global__ void __launch_bounds__(kThreads, kResident<DT, PAGED>)
     }
     __syncwarp();  // the angles may be written again
   }
+  // rows beyond the packed ones, whose keys are missing (nobody waits for this load)
+  if constexpr (PAGED) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.batch.q_start[a.batch.s] > a.batch.n)
+      record_device_error(MOSS_ERR_VALUE);
+  }
 }
 
 template <int DT, int D, bool PAGED, bool PAIRS>

@@ -19,6 +19,9 @@ of query heads, and heads are 64 or 128 wide.
 
 The index tensors stay on the device, so a captured call can be replayed
 with other lengths, tables and row counts in them.
+What they say wrongly (a page outside the pool, a position outside the table,
+for `rope_paged_kv` a row beyond the packed ones) is left out and reported
+through the device error word.
 """
 
 import torch

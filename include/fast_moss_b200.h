@@ -300,8 +300,10 @@ MOSS_API int moss_qk_norm_rope(const void* q, const void* k, int dtype, const fl
  * All index arrays live on the device and are read there, so a captured call
  * can be replayed with other lengths, tables and row counts.  A page outside
  * the pool, or a position outside the table, is not touched and is reported
- * by moss_check_device_error; other sequences are not affected.  Sequences may
- * share pages (a common beginning) that no new token falls into.
+ * by moss_check_device_error; other sequences are not affected.  Where q_start
+ * passes n the rows that are there keep their positions, and moss_rope_paged_kv
+ * reports that keys are missing.  Sequences may share pages (a common beginning)
+ * that no new token falls into.
  *
  * moss_rope_paged_kv: the new tokens' queries rotated (normed first where
  * q_weight / k_weight are given, as moss_qk_norm_rope) into oq [n, hq, d]

@@ -751,3 +751,27 @@ def test_wide_groups_of_query_heads(moss, cuda_device, hq, hkv, d):
                                        max_tokens=hint)
             check_attention(got, want, size, 13 * (hq // hkv))
     no_device_error()
+
+
+@pytest.mark.parametrize("t", [4, 50])
+def test_rows_beyond_the_packed_ones_are_reported(moss, cuda_device, t):
+    """Index tensors that promise more rows than there are: the rows that are
+    there are what they would be beside the others, and the append, whose keys
+    are missing, sets the error word; also where a whole sequence is missing."""
+    from fast_moss_b200 import _lib
+
+    no_device_error()
+    for n in (2 * t - 3, t):
+        h = History([t, t], [100, 30], 2, 64, 16, cuda_device, seed=t)
+        x = torch.randn(h.n, 6, 64, device=cuda_device, dtype=torch.bfloat16)
+        q = moss.rope_paged_kv(x[:, :2], x[:, 2:4], x[:, 4:], *h.index, PERIOD, h.k, h.v)
+        want, size = attention_reference(h, q, 0, 1 / 8)
+        no_device_error()
+        k, v = h.k.clone(), h.v.clone()
+        part = moss.rope_paged_kv(x[:n, :2], x[:n, 2:4], x[:n, 4:], *h.index, PERIOD, k, v)
+        assert take_device_error() == _lib.ERR_TIMEOUT
+        assert torch.equal(part, q[:n]) and torch.equal(k, h.k) and torch.equal(v, h.v)
+        for hint in (None, t):
+            got = moss.paged_attention(q[:n], h.k, h.v, *h.index, max_tokens=hint)
+            check_attention(got, want[:n], size[:n], t)
+    no_device_error()

@@ -201,3 +201,19 @@ def test_wrappers_refuse_tensors_that_are_not_on_a_gpu():
         fm.paged_attention(x, pages, pages, *index)
     with pytest.raises(ValueError):
         fm.rope_paged_kv(x, x[:, :1], x[:, :1], *index, 1e4, pages, pages)
+
+
+@pytest.mark.parametrize("rows,tile", [(16, 64), (256, 128)])
+def test_rows_that_are_there_keep_their_positions(rows, tile):
+    """A sequence with more rows than were packed: row r is position kv_len -
+    (q_start[s + 1] - r) all the same, where rope_paged_kv put it."""
+    (p,) = plan([0, 10], [100], 6, rows=rows, tile=tile, ctas=1)
+    assert p[6:8] == (0, 96)  # the last row that is there, 5, is position 95
+    (p,) = plan([0, 10], [100], 6, rows=rows, tile=tile, ctas=1, context=20)
+    assert p[6:8] == (71, 96)
+    (p,) = plan([0, 10], [3], 6, rows=rows, tile=tile, ctas=1)  # all before position 0
+    assert p[6:8] == (0, 0)
+    first, = plan([0, 6, 10], [50, 60], 6, rows=rows, tile=tile, ctas=1)
+    assert first[6:8] == (0, 50)
+    (p,) = plan([0, 2 ** 63 - 1], [2 ** 63 - 1], 6, rows=rows, tile=tile, ctas=1)
+    assert 0 <= p[6] <= p[7] <= 128
