@@ -704,7 +704,7 @@ int run(Args& a, int64_t most, void* workspace, cudaStream_t stream,
     a.split.min_q = few ? kFewRows + 1 : 1;
     a.split.max_q = 0x7fffffff;
     a.split.setup = kTcSetup;
-    a.least = 1 + kTcSetup;
+    a.least = 1 + kTcSetup;  // a tile at least
     place(a, workspace, space(ctas, kTcRows, D));
     status = launch_tc(a, D, ctas, stream, name);
   }
@@ -794,6 +794,11 @@ extern "C" int64_t moss_paged_attention_plan(const int64_t* q_start, const int64
       tile < 1 || setup < 0 || (rows & (rows - 1)) || (tile & (tile - 1)) || ctas < 1 ||
       page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
     return -1;
+  // as moss_paged_attention, whose index arithmetic this is
+  if (group > (1 << 20) || hkv > (1 << 20) / group || n > 0x3fffffff / group || s > 0x3fffffff ||
+      max_pages < 0 || max_pages > 0x7ffffeff / page_size || context < 0 || rows > (1 << 20) ||
+      tile > (1 << 20) || setup > (1 << 20) || ctas > (1 << 24))
+    return -1;
   paged::Batch b{};
   b.q_start = q_start;
   b.kv_len = kv_len;
@@ -812,7 +817,8 @@ extern "C" int64_t moss_paged_attention_plan(const int64_t* q_start, const int64
   w.setup = static_cast<int>(setup);
   int64_t total = 0;
   for (int i = 0; i < b.s; ++i) total += hkv * paged::head_work(w, paged::load_seq(b, i));
-  const int64_t share = paged::share_of(total, static_cast<int>(ctas), 1 + w.setup);
+  const int least = (tile == pattn::kGroup ? pattn::kLeastGroups : 1) + w.setup;
+  const int64_t share = paged::share_of(total, static_cast<int>(ctas), least);
   int64_t count = 0;
   for (int64_t c = 0; c < ctas; ++c) {
     const int64_t begin = share * c;

@@ -330,13 +330,22 @@ MOSS_API int moss_qk_norm_rope(const void* q, const void* k, int dtype, const fl
  * 2^-8 of each weight).  Sums are float32 in a fixed order for given lengths
  * (deterministic).
  *
- * moss_paged_attention_plan: the work split of moss_paged_attention for host
- * copies of the index arrays (no device needed), for blocks of `rows` rows,
- * tiles of `tile` keys (powers of two) and items that cost `setup` tiles before
- * their first over `ctas` workers: for every piece of work 9 int64 (cta, sequence, key head, row block, first tile, tiles, first key of
- * the block, end of its keys, 1 if it begins the block's keys + 2 if it ends
- * them).  Returns the number of pieces (at most max_pieces are written), -1
- * for bad arguments.  For tests and capacity planning.
+ * moss_paged_attention_plan: how one of moss_paged_attention's kernels splits its
+ * work, for host copies of the index arrays (no device needed): blocks of `rows`
+ * rows, tiles of `tile` keys (powers of two), items that cost `setup` tiles before
+ * their first, `ctas` workers.  The kernels' own figures are
+ *   at most 8 rows per key head       rows 8,   tile 16,  setup 2
+ *   few rows                          rows 16,  tile 16,  setup 2
+ *   many rows                         rows 256, tile 128, setup 3
+ * with a worker a multiprocessor for many rows, and for few 16 (d = 64), 12 (d =
+ * 128, blocks of 8) or 8 (d = 128, blocks of 16) a multiprocessor.  A worker takes
+ * setup + 1 tiles at least, setup + 2 of 16 keys.  Where a batch goes to both
+ * kernels, each splits its own sequences: give the others no rows.  For every
+ * piece of work 9 int64 (worker, sequence, key head, row block, first tile, tiles,
+ * first key of the block, end of its keys, 1 if it begins the block's keys + 2 if
+ * it ends them).  Returns the number of pieces (at most max_pieces are written),
+ * -1 for bad arguments, the sizes that moss_paged_attention refuses among them.
+ * For tests and capacity planning.
  * ------------------------------------------------------------------------- */
 MOSS_API int moss_rope_paged_kv(const void* q, const void* k, const void* v, int dtype,
               const float* q_weight, const float* k_weight, float eps, const int64_t* q_start,

@@ -217,3 +217,57 @@ def test_rows_that_are_there_keep_their_positions(rows, tile):
     assert first[6:8] == (0, 50)
     (p,) = plan([0, 2 ** 63 - 1], [2 ** 63 - 1], 6, rows=rows, tile=tile, ctas=1)
     assert 0 <= p[6] <= p[7] <= 128
+
+
+@pytest.mark.parametrize("seed", range(12))
+@pytest.mark.parametrize("rows,tile,setup,least", [(8, 16, 2, 4), (16, 16, 2, 4), (256, 128, 3, 4)])
+def test_the_split_of_the_kernels_own_shapes(rows, tile, setup, least, seed):
+    """Blocks, tiles, set-up and least share as the three forms of the kernels
+    have them: every key of every block once, shares that are even."""
+    rng = random.Random(seed)
+    group, hkv = rng.choice([1, 2, 5]), rng.choice([1, 3])
+    context = rng.choice([0, 0, 30, 200])
+    ctas = rng.choice([3, 148, 148 * 12])
+    most = 32 // group if rows < 256 else 700
+    new = [rng.choice([0, 1, 1, 4, rng.randint(0, most)]) for _ in range(rng.randint(1, 9))]
+    past = [rng.choice([0, 1, 15, 16, 17, 255, 256, rng.randint(0, 3000)]) for _ in new]
+    length = [a + b for a, b in zip(new, past)]
+    q_start = [sum(new[:i]) for i in range(len(new) + 1)]
+    pieces = plan(q_start, length, q_start[-1], group=group, hkv=hkv, columns=400, context=context,
+                  rows=rows, tile=tile, setup=setup, ctas=ctas)
+    items = {}
+    for p in pieces:
+        items.setdefault(p[1:4], []).append(p)
+    total = sum(p[5] for p in pieces) + setup * len(items)
+    share = max(-(-total // ctas), least)
+    assert set(items) == {(s, h, b) for s, t in enumerate(new) for h in range(hkv)
+                          for b in range(-(-t * group // rows))}
+    at = 0  # tiles before the item, its set-up among them
+    for s, h, b in sorted(items):
+        seen = keys_of(new[s], length[s], group, context, rows, b)
+        tiles = -(-(max(seen) + 1) // tile) - min(seen) // tile
+        expected, k = [], at
+        while k < at + setup + tiles:
+            end = min((k // share + 1) * share, at + setup + tiles)
+            first, last = max(k - at - setup, 0), end - at - setup
+            if last > first:
+                expected.append((k // share, first, last - first))
+            k = end
+        assert [(p[0], p[4], p[5]) for p in items[s, h, b]] == expected
+        at += setup + tiles
+
+
+def test_plan_refuses_what_the_attention_refuses():
+    """Sizes beyond the kernels' index arithmetic."""
+    lib = _lib.load()
+    z = _lib.strides([0, 0])
+
+    def ask(n=1, s=1, group=1, hkv=1, page=16, columns=1, rows=16, tile=64, setup=0, ctas=1):
+        return lib.moss_paged_attention_plan(z, z, n, s, group, hkv, page, columns, 0, rows, tile,
+                                             setup, ctas, z, 0)
+
+    assert ask(s=0) == 0
+    for kw in (dict(n=1 << 30), dict(n=1 << 20, group=1 << 11), dict(s=1 << 30), dict(hkv=1 << 21),
+               dict(columns=1 << 28), dict(columns=-1), dict(rows=1 << 31), dict(tile=1 << 31),
+               dict(setup=1 << 31), dict(ctas=1 << 31)):
+        assert ask(**kw) == -1, kw
