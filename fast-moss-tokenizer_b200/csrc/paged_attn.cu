@@ -630,12 +630,12 @@ void place(Args& a, void* workspace, const Space& s) {
 // Query rows per key head above which a sequence goes to the tensor-memory
 // kernel, whose blocks of 256 rows cost the same however few are used: 64
 // streams of 24 rows in a window of 250 37 us here, 77 there, of 64 rows 62 and
-// 87; 16 streams of 32 rows over 2000 keys 69 and 68, of 64 rows 106 and 73.
+// 87; 16 streams of 32 rows over 2000 keys 69 and 68, of 64 rows 106 and 73.  The
+// border is also where the weights go from two bf16 terms to one, so it looks at
+// the sequence's own rows, not at its neighbours: a sequence by itself is in part
+// faster there from 16 rows on (32 rows over 2000 keys 18 us here, 15 there, over
+// 30,000 60 and 54; 16 rows 17 and 15, 42 and 53).
 constexpr int kFewRows = 32;
-// A sequence by itself leaves the device idle anyhow, and the fewer, longer runs
-// of the other kernel are joined sooner: 32 rows over 2000 keys 18 us here, 15
-// there, over 30,000 60 and 54; 16 rows 17 and 15, but over 30,000 42 and 53.
-constexpr int kFewRowsAlone = 16;
 // Rows for which the narrow form of the kernel (8 rows a block, more warps) is
 // taken: 4 rows in a window of 250 20 us, 24 in the wide form.
 constexpr int kNarrowRows = 8;
@@ -684,11 +684,11 @@ int launch_rows(Args& a, void* workspace, cudaStream_t stream, const char* name)
 
 // most: bound of the rows per key head of any sequence.  Sequences of few rows
 // and longer ones each have their kernel; where the bound allows both, both run
-// and each takes its own.  A single sequence has one kind only.
+// and each takes its own.  A single sequence has one kind only, the bound's.
 template <int D>
 int run(Args& a, int64_t most, void* workspace, cudaStream_t stream,
         const char* name) {
-  const bool many = most > (a.batch.s > 1 ? kFewRows : kFewRowsAlone);
+  const bool many = most > kFewRows;
   const bool few = !many || a.batch.s > 1;
   int status = MOSS_OK;
   if (few) {
@@ -727,7 +727,7 @@ using namespace moss;
 
 extern "C" int64_t moss_paged_attention_workspace(int64_t d, int64_t rows) {
   if (d != 64 && d != 128) return 0;
-  const bool many = rows > pattn::kFewRowsAlone;
+  const bool many = rows > pattn::kFewRows;
   return d == 64 ? pattn::workspace_bytes<64>(many) : pattn::workspace_bytes<128>(many);
 }
 

@@ -325,9 +325,9 @@ MOSS_API int moss_qk_norm_rope(const void* q, const void* k, int dtype, const fl
  * moss_paged_attention_workspace(d, rows) bytes, rows = (max_tokens, or n if 0
  * or larger) * (hq / hkv); 16-byte aligned, contents irrelevant before and
  * after; calls that may overlap in time need one each.  Sequences with at most
- * 16 rows per key head (32 in a batch of several) keep their weights in two
- * bf16 terms (2^-16 relative), longer ones may round them to bf16 (half a step:
- * 2^-8 of each weight).  Sums are float32 in a fixed order for given lengths
+ * 32 rows per key head keep their weights in two bf16 terms (2^-16 relative),
+ * longer ones may round them to bf16 (half a step: 2^-8 of each weight); a
+ * sequence by itself counts as `rows` rows.  Sums are float32 in a fixed order for given lengths
  * (deterministic).
  *
  * moss_paged_attention_plan: how one of moss_paged_attention's kernels splits its

@@ -93,3 +93,46 @@ def test_leaping_scores(moss, cuda_device, d, new, past, hq, hkv, context):
     check(h, q, got, context, max(new) * (hq // hkv) > 16)
     again = moss.paged_attention(q, h.k, h.v, *h.index, scale=SCALE, context=context or None)
     assert torch.equal(again, got)
+
+
+def cancelling(h, hq, g):
+    """Queries and values whose results are zero but for rounding: the earlier
+    keys' values, taken by their weights, cancel, and the new tokens' keys score
+    50 below all others, so that every row of a sequence has the same weights.
+    What is left of a result is the error of the weights."""
+    hkv, d = h.k.shape[1], h.k.shape[3]
+    q = torch.zeros(h.n, hq, d, device=h.k.device, dtype=torch.bfloat16)
+    for s, t in enumerate(h.new):
+        u = torch.randn(hkv, d, generator=g).to(h.k.device, torch.bfloat16)
+        q[h.start[s]:h.start[s] + t] = u.repeat_interleave(hq // hkv, 0)
+        page, slot = h.where(s, torch.arange(h.past[s], h.length[s], device=h.k.device))
+        h.k[page, :, slot] = (-60 * d ** 0.5 / u.float().pow(2).sum(-1, keepdim=True) * u).to(
+            torch.bfloat16)
+        k, v = h.dense(s)
+        weight = torch.softmax(torch.einsum("hd,hkd->hk", u.double(), k) * d ** -0.5, -1)
+        mean = torch.einsum("hk,hkd->hd", weight, v)
+        page, slot = h.where(s, torch.arange(h.past[s], device=h.k.device))
+        h.v[page, :, slot] = (h.v[page, :, slot].double() - mean).to(torch.bfloat16)
+    return q
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [[1], [8], [9], [16], [17], [25], [32], [33],
+                                 [32, 1, 17, 8], [1, 200, 9, 32, 16, 33, 2]])
+def test_weights_in_two_terms(moss, cuda_device, new, d):
+    """The weights of a sequence of up to 32 rows per key head are good to 2^-16,
+    alone as beside others, longer ones among them; beyond, to 2^-8."""
+    hkv = 3
+    g = torch.Generator().manual_seed(d)
+    h = History(new, [90 + 11 * i for i in range(len(new))], hkv, d, 16, cuda_device, seed=d)
+    q = cancelling(h, hkv, g)
+    want, size = attention_reference(h, q, 0, d ** -0.5)
+    for hint in (None, max(new)):
+        got = moss.paged_attention(q, h.k, h.v, *h.index, max_tokens=hint)
+        no_device_error()
+        for s, t in enumerate(new):
+            rows = slice(h.start[s], h.start[s] + t)
+            weight = 2.0 ** -15 + (2.0 ** -8 if t > 32 else 0.0)
+            bound = (2.0 ** -8 * want[rows].abs() + weight * size[rows]) * 1.001
+            worst = ((got[rows].double() - want[rows]).abs() / bound).max().item()
+            assert worst <= 1.0, (t, worst)
