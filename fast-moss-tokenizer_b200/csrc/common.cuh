@@ -45,7 +45,8 @@ __device__ __forceinline__ void record_device_error(int code) {
 
 // ---------------------------------------------------------------- bounded waits
 // Every spin in these kernels (on an mbarrier phase, a copy or an MMA) goes
-// through bounded_wait: it polls until `poll()` is true, and after
+// through bounded_wait (or, in paged_attn_tc.cu, through a wait of its own that
+// ends in the same way): it polls until `poll()` is true, and after
 // `limit_ns` of %globaltimer time gives up, records MOSS_ERR_TIMEOUT in the
 // device error word and returns false.  The caller then stops issuing work,
 // waits (bounded again) for its own copies in flight, frees what it holds

@@ -250,9 +250,10 @@ __device__ __forceinline__ bool test_phase(uint32_t bar, uint32_t parity) {
 }
 // SUSPEND: the instruction that may suspend the thread for a while, for waits
 // off the critical path, whose polling would take issue slots from the softmax.
+constexpr uint32_t kWaitLimit = static_cast<uint32_t>(kWaitLimitNs >> 20);
 template <bool SUSPEND>
 __device__ __forceinline__ void wait_phase(unsigned long long* bar, uint32_t parity,
-                                           volatile int* gave_up) {
+                                           volatile int* gave_up, uint32_t limit = kWaitLimit) {
   const uint32_t at = pipe::smem_u32(bar);
   parity &= 1;
   uint32_t start = 0;
@@ -263,7 +264,7 @@ __device__ __forceinline__ void wait_phase(unsigned long long* bar, uint32_t par
       const uint32_t now = static_cast<uint32_t>(global_ns() >> 20);  // about a millisecond
       if (start == 0) start = now;
       if (*gave_up) return;
-      if (now - start > static_cast<uint32_t>(kWaitLimitNs >> 20)) {
+      if (now - start > limit) {
         *gave_up = 1;
         record_device_error(MOSS_ERR_TIMEOUT);
         return;
@@ -1066,6 +1067,30 @@ __global__ void __launch_bounds__(kTcRows) join_kernel(const __grid_constant__ A
   dst[1] = pack_bf16x8(v + 8);
 }
 
+// Two warps in two waits each, one polling and one suspending, on phases that are
+// completed beforehand (arrive) or never: the first wait to run out ends the others.
+__global__ void wait_probe_kernel(uint32_t limit, int arrive) {
+  __shared__ unsigned long long bars[2];
+  __shared__ int gave_up;
+  if (threadIdx.x == 0) {
+    pipe::mbar_init(&bars[0], 1);
+    pipe::mbar_init(&bars[1], 1);
+    gave_up = 0;
+    pipe::fence_mbar_init();
+  }
+  __syncthreads();
+  if (arrive && threadIdx.x == 0) {
+    pipe::mbar_arrive(&bars[0]);
+    pipe::mbar_arrive(&bars[1]);
+  }
+  for (int i = 0; i < 2; ++i) {
+    if (threadIdx.x < 32)
+      wait_phase<false>(&bars[i], 0, &gave_up, limit);
+    else
+      wait_phase<true>(&bars[i], 0, &gave_up, limit);
+  }
+}
+
 template <int D>
 int launch(const Args& a, int ctas, cudaStream_t stream, const char* name) {
   TcArgs args{};
@@ -1127,3 +1152,12 @@ int launch_tc(const Args& a, int64_t d, int ctas, cudaStream_t stream, const cha
 
 }  // namespace pattn
 }  // namespace moss
+
+extern "C" int moss_test_paged_wait(int64_t limit_ns, int arrive, void* stream) {
+  const char* name = "moss_test_paged_wait";
+  if (limit_ns < 1000 || limit_ns > 100000000)
+    return moss::fail(MOSS_ERR_VALUE, "%s: limit must be 1 us to 100 ms", name);
+  moss::pattn::wait_probe_kernel<<<1, 64, 0, moss::as_stream(stream)>>>(
+      static_cast<uint32_t>(limit_ns >> 20), arrive ? 1 : 0);
+  return moss::launch_status(name);
+}

@@ -85,6 +85,11 @@ MOSS_API int moss_check_device_error(void* stream);
  * usable.  Stream-ordered; for tests. */
 MOSS_API int moss_test_bounded_wait(int64_t limit_ns, int arrive, void* stream);
 
+/* The same for the waits of moss_paged_attention's kernel for many rows, which
+ * poll or suspend and, once one has run out, all return at once: two warps, one
+ * of either kind, wait twice each.  Limits count in milliseconds (2^20 ns). */
+MOSS_API int moss_test_paged_wait(int64_t limit_ns, int arrive, void* stream);
+
 /* ---------------------------------------------------------------------------
  * Residual update with per-channel layer scale.
  * Replaces fast_moss/v2_pointwise.py:92-122 (`_scale_add` / `scale_add`):

@@ -271,3 +271,8 @@ def test_plan_refuses_what_the_attention_refuses():
                dict(columns=1 << 28), dict(columns=-1), dict(rows=1 << 31), dict(tile=1 << 31),
                dict(setup=1 << 31), dict(ctas=1 << 31)):
         assert ask(**kw) == -1, kw
+
+
+@pytest.mark.parametrize("limit", [0, 999, 100_000_001, -5])
+def test_wait_limits_out_of_range_are_refused(limit):
+    assert _lib.load().moss_test_paged_wait(limit, 1, None) == _lib.ERR_VALUE
