@@ -174,9 +174,12 @@ class PagedHistory:
 
     def reset(self, sequences=None):
         """Starts the given sequences (all by default) afresh; their pages go
-        back to the pool."""
-        for s in range(self.sequences) if sequences is None else sequences:
+        back to the pool.  Raises ValueError, with nothing changed, where one does
+        not exist."""
+        sequences = list(range(self.sequences) if sequences is None else sequences)
+        for s in sequences:
             if not 0 <= s < self.sequences:
                 raise ValueError(f"no sequence {s}")
+        for s in sequences:
             self._give_back(s, list(self._pages[s]))
             self.lengths[s] = 0

@@ -134,3 +134,17 @@ def test_a_step_takes_at_least_the_rows_that_were_made_room_for():
     with pytest.raises(RuntimeError, match="pages"):
         h.advance([59, 62])
     assert h.rows == 1
+
+
+def test_a_refused_reset_changes_nothing():
+    h = history(pages=6, max_positions=64)
+    h.advance([20, 10, 33])
+    state = (list(h.lengths), h.free_pages)
+    for bad in ([0, 3], [1, -1], [2, 0, 99], iter([0, 5])):
+        with pytest.raises(ValueError):
+            h.reset(bad)
+        assert (h.lengths, h.free_pages) == state
+    h.reset(iter([2, 0, 2]))  # the same one twice
+    assert h.lengths == [0, 10, 0] and h.free_pages == 5
+    h.advance([0, 1, 0])
+    check(h, [0, 0, 0])
