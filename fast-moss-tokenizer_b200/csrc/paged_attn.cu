@@ -432,16 +432,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::warps * 32, 1)
         for (int d = 4; d < 32; d <<= 1)
           l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
       if (whole) {
-        float inv[2];  // a row that attends to nothing is zero
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          inv[e] = l[nt][e] > 0.0f || l[nt][e] != l[nt][e] ? 1.0f / l[nt][e] : 0.0f;
+        const float inv[2] = {inverse_of(l[nt][0]), inverse_of(l[nt][1])};
 #pragma unroll
         for (int i = 0; i < kKs; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t x = transpose8(
-                pack_bf16x2(o[i][nt][2 * j] * inv[0], o[i][nt][2 * j + 1] * inv[1]));
+                pack_bf16x2(normed(o[i][nt][2 * j], inv[0]), normed(o[i][nt][2 * j + 1], inv[1])));
             if (8 * nt + row < rows)
               *reinterpret_cast<uint32_t*>(a.out + row_at[nt] + i * 16 + j * 8 + pair) = x;
           }
@@ -549,13 +546,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     return sum;
   };
   auto put = [&](const Note& n, const Sum& sum, int r) {
-    const float inv = sum.l > 0.0f || sum.l != sum.l ? 1.0f / sum.l : 0.0f;
+    const float inv = inverse_of(sum.l);
     const int rr = (n.block << a.split.rows_shift) + r;
     const int t = paged::quotient(rr, a.split.group);
     uint16_t* dst = a.out + ((static_cast<int64_t>(n.row0) + t) * a.hq + n.h * group +
                              (rr - t * group)) * D + col * 4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(sum.v.x * inv, sum.v.y * inv),
-                                                pack_bf16x2(sum.v.z * inv, sum.v.w * inv));
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack_bf16x2(normed(sum.v.x, inv), normed(sum.v.y, inv)),
+                   pack_bf16x2(normed(sum.v.z, inv), normed(sum.v.w, inv)));
   };
   auto pieces_of = [&](const Note& n, int first) {
     return n.state == 0 || n.last < first || n.last >= workers ? 0 : n.last - first + 1;

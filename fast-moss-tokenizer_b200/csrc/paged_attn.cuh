@@ -241,6 +241,16 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
+// A row's values are its sums times 1 / l; of a row that attends to nothing (l = 0)
+// zeros, whatever the sums hold: a weight of zero times an infinity that other rows
+// of the block attend to is NaN.
+__device__ __forceinline__ float inverse_of(float l) {
+  return l > 0.0f || l != l ? 1.0f / l : 0.0f;
+}
+__device__ __forceinline__ float normed(float sum, float inverse) {
+  return inverse == 0.0f ? 0.0f : sum * inverse;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

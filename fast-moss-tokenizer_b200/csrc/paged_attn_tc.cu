@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // ---- this row's result
       const bool any = from < to;
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const float inv = inverse_of(l);
       if (!whole && row_on) a.stats[slot * kTcRows + w * kTileRows + r] = make_float2(m, l);
       // cut pieces: [d / 4][rows] of four values, so that a warp's rows lie side
       // by side
@@ -981,7 +981,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float f[8];
 #pragma unroll
               for (int x = 0; x < 8; ++x)
-                f[x] = inv == 0.0f ? 0.0f : __uint_as_float(o[e + x]) * inv;
+                f[x] = normed(__uint_as_float(o[e + x]), inv);
               dst[e / 8] = pack_bf16x8(f);
             }
           } else {
@@ -1054,9 +1054,9 @@ __global__ void __launch_bounds__(kTcRows) join_kernel(const __grid_constant__ A
       }
     }
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const float inv = inverse_of(l);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) v[e] = inv == 0.0f ? 0.0f : v[e] * inv;
+  for (int e = 0; e < 16; ++e) v[e] = normed(v[e], inv);
   const int rr = n.block * kTcRows + row;
   const int t = paged::quotient(rr, a.split.group);
   const int group = static_cast<int>(a.split.group.d);

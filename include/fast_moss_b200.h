@@ -323,7 +323,9 @@ MOSS_API int moss_qk_norm_rope(const void* q, const void* k, int dtype, const fl
  * head h / (hq / hkv).  q [n, hq, d] and out [n, hq, d]: bf16, contiguous.
  * A row that attends to nothing (a sequence with more new tokens than
  * positions) is zero.  Keys and values that no row of a sequence attends to
- * have no effect, whatever they hold.  max_tokens: an upper bound of any
+ * have no effect, whatever they hold; a value that is not finite and that some
+ * rows attend to may also make others of the same sequence NaN (a weight of zero
+ * does not silence it).  max_tokens: an upper bound of any
  * sequence's new tokens if the caller knows one, else 0; it chooses between
  * kernels and never changes what is computed beyond rounding (a sequence with
  * more is computed all the same).  workspace: at least

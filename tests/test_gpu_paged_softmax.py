@@ -136,3 +136,42 @@ def test_weights_in_two_terms(moss, cuda_device, new, d):
             bound = (2.0 ** -8 * want[rows].abs() + weight * size[rows]) * 1.001
             worst = ((got[rows].double() - want[rows]).abs() / bound).max().item()
             assert worst <= 1.0, (t, worst)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("t,length", [(3, 1), (8, 5), (32, 31), (60, 50)])
+def test_rows_without_a_position_beside_values_that_are_not_finite(moss, cuda_device, t, length,
+                                                                   bad, d):
+    """A sequence with more new tokens than positions: its first rows are zero
+    whatever the others attend to, in whole pieces and in joined ones."""
+    h = History([t] * 3, [0] * 3, 7, d, 16, cuda_device)
+    h.kv_len.fill_(length)
+    h.v.fill_(bad)
+    q = torch.randn(h.n, 7, d, device=cuda_device, dtype=torch.bfloat16)
+    for hint in (None, t):
+        got = moss.paged_attention(q, h.k, h.v, *h.index, max_tokens=hint).view(3, t, 7, d)
+        assert torch.equal(got[:, :t - length], torch.zeros_like(got[:, :t - length]))
+        assert not torch.isfinite(got[:, t - length:].float()).any()
+    no_device_error()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [[3, 2], [20, 16], [40, 20], [300, 129]])
+def test_masked_places_have_no_effect(moss, cuda_device, new, d):
+    """Infinities, NaN and the type's extremes in keys and values that no row of
+    a sequence attends to, for both widths of head and all forms of the kernels."""
+    past, context = [400, 190], 150
+    outs = []
+    for poison in (0.0, float("nan"), float("inf"), -float("inf"), torch.finfo(torch.bfloat16).min):
+        h = History(new, past, 3, d, 32, cuda_device, seed=3, poison=poison)
+        for s in range(2):  # positions before every row's window
+            page, slot = h.where(s, torch.arange(0, past[s] - context + 1, device=cuda_device))
+            h.k[page, :, slot] = poison
+            h.v[page, :, slot] = poison
+        g = torch.Generator().manual_seed(4)
+        q = torch.randn(h.n, 6, d, generator=g).to(cuda_device, torch.bfloat16)
+        outs.append(moss.paged_attention(q, h.k, h.v, *h.index, context=context))
+    no_device_error()
+    assert torch.isfinite(outs[0].float()).all()
+    assert all(torch.equal(o, outs[0]) for o in outs)
