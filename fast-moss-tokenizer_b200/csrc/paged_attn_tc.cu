@@ -75,6 +75,11 @@ constexpr uint32_t kSub = kKeys * 128;  // 128 rows x 64 columns of bf16
 constexpr uint32_t kTmemCols = 512;
 
 constexpr float kSlack = 8.0f;
+// d = 128: the sum of a tile's weights above which the reference is raised by a power
+// of two before the next tile, and the sum above which the tile is done again by its
+// true maximum.  Between the two a tile's products are formed with weights that
+// large, so the second leaves float32 sums room for values up to 2^55.
+constexpr float kRaiseAbove = 0x1p16f, kRedoAbove = 0x1p64f;
 // Tiles that would run in step (each finds its next scores ready, d = 64) and
 // leave the special-function unit idle between the exponentials take turns
 // instead: one's loads and stores lie behind the other's exponentials.
@@ -931,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           weights();
           if (turns && (w == 0 || j + 1 < steps)) turn_pass(w ^ 1);
           if (!kOwnP<D>) {
-            if (__any_sync(0xffffffffu, !(sum < 0x1p100f))) {
+            if (__any_sync(0xffffffffu, !(sum < kRedoAbove))) {
               // scores far above the reference (or not finite): take the true
               // maximum and do the tile again (its scores are still there)
               load_scores();
@@ -939,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               weights();
             }
             const int exponent = static_cast<int>(__float_as_uint(sum) >> 23) - 127;
-            raise = sum > 0x1p16f ? static_cast<float>(exponent) : 0.0f;
+            raise = sum > kRaiseAbove ? static_cast<float>(exponent) : 0.0f;
           } else if (j > from) {
             // the product before has read the weights that these replace
             wait(&bars.pv_done[w], seen - 1);

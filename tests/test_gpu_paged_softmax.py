@@ -4,7 +4,7 @@ tile, against plain float64 evaluations.
 The kernels take weights against a reference that they move late: by the
 running maximum once it is exceeded by 2^8 (few rows; d = 64), or raised by a
 power of two when a tile's weights passed 2^16 and by the true maximum when
-they passed 2^100 (d = 128, many rows).  Every such path is reached here: rows
+they passed 2^64 (d = 128, many rows).  Every such path is reached here: rows
 of all kinds lie side by side in one warp, so that a step takes several of
 them at once.
 
@@ -26,7 +26,7 @@ pytestmark = pytest.mark.gpu
 PROFILES = [
     [0] * 12,
     [0, 30, 30, 30, 30, 30, 30, 30, 30, 30, 30, 30],            # passes 2^16 once
-    [0, 0, 130, 130, 130, 130, 130, 130, 130, 130, 130, 130],   # passes 2^100 once
+    [0, 0, 130, 130, 130, 130, 130, 130, 130, 130, 130, 130],   # passes 2^64 once
     [0, 22, 44, 66, 88, 110, 132, 154, 176, 198, 220, 242],     # 2^16 in every tile
     [0, 120, 0, 0, 120, 121, 0, 0, 0, 120, 0, 121],             # up and down again
     [0, 126, 252, 252, 252, 252, 252, 252, 252, 252, 252, 252],
@@ -175,3 +175,24 @@ def test_masked_places_have_no_effect(moss, cuda_device, new, d):
     no_device_error()
     assert torch.isfinite(outs[0].float()).all()
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("leap", [15, 17, 40, 63, 65, 90, 101])
+@pytest.mark.parametrize("new", [[5], [200]])
+def test_leaps_over_large_values(moss, cuda_device, new, leap, d):
+    """Values of 2^40 and a leap of the scores in one tile, of any size: the sums
+    that hold both stay finite, as the results are."""
+    g = torch.Generator().manual_seed(leap)
+    h = History(new, [700], 2, d, 32, cuda_device, seed=leap)
+    q = torch.zeros(h.n, 2, d, device=cuda_device)
+    q[..., 0] = 1
+    q[..., 1:] = 0.3 / SCALE / d ** 0.5 * torch.randn(h.n, 2, d - 1, generator=g).to(cuda_device)
+    q = q.to(torch.bfloat16)
+    at = torch.arange(h.length[0], device=cuda_device)
+    page, slot = h.where(0, at)
+    h.k[page, :, slot, 0] = torch.where(at < 400, 0.0, float(leap)).to(torch.bfloat16)[:, None]
+    h.v.mul_(2.0 ** 40)
+    got = moss.paged_attention(q, h.k, h.v, *h.index, scale=SCALE)
+    no_device_error()
+    check(h, q, got, 0, new[0] > 16)
