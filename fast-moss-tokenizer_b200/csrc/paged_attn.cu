@@ -26,7 +26,7 @@
 //
 // Measured: 61 single tokens over up to 8000 positions (32 heads over 8 of 128,
 // 315 MB) 61 us, 5160 GB/s or 0.79 of a plain copy; one token over 131,000
-// positions 94 us, 0.87; 64 streams of 4 tokens in a window of 250 (55 MB) 20 us,
+// positions 94 us, 0.87; 64 streams of 4 tokens in a window of 250 (55 MB) 19 us,
 // of which 6 until the first keys arrive and 9 steps of half a microsecond after
 // them; one stream of 4 tokens over 2000 positions 13 us, the same latencies.
 //
@@ -631,8 +631,10 @@ void place(Args& a, void* workspace, const Space& s) {
 // 87; 16 streams of 32 rows over 2000 keys 69 and 68, of 64 rows 106 and 73.  The
 // border is also where the weights go from two bf16 terms to one, so it looks at
 // the sequence's own rows, not at its neighbours: a sequence by itself is in part
-// faster there from 16 rows on (32 rows over 2000 keys 18 us here, 15 there, over
-// 30,000 60 and 54; 16 rows 17 and 15, 42 and 53).
+// faster there from 16 rows on (32 rows over 2000 keys 17 us here, 15 there, over
+// 30,000 56 and 53; 16 rows 17 and 15, 42 and 53).  Rows are only half of what
+// parts the kernels in time, keys a block the other: in a short window 64 rows are
+// still faster here, over long histories 32 already there.
 constexpr int kFewRows = 32;
 // Rows for which the narrow form of the kernel (8 rows a block, more warps) is
 // taken: 4 rows in a window of 250 20 us, 24 in the wide form.

@@ -29,9 +29,9 @@
 // What bounds it: a step of 256 rows x 128 keys is 32768 exponentials, 2048
 // clocks of an SM's 16 a clock, against 1024 (d = 64) or 2048 (d = 128) clocks
 // of tensor-core time.  2048 tokens over 14,300 positions, 20 heads: d = 64
-// 238 us, 675 TF/s, about 2800 clocks a step: a tile's exponentials 1400 (1024 at
+// 232 us, 693 TF/s, about 2800 clocks a step: a tile's exponentials 1400 (1024 at
 // the full rate, one warp a scheduler at a time), its loads, maximum, stores and
-// barriers as long, behind the other tile's exponentials; d = 128 312 us, 1030
+// barriers as long, behind the other tile's exponentials; d = 128 309 us, 1040
 // TF/s, about 3950 clocks a step, the chain of one tile's weights (2300) and the
 // two products after them (1060, and 600 between the issue of one and the sight
 // of the other's end).
